@@ -779,6 +779,7 @@ struct Attend {
       }
       if (!ok) return;
       uint32_t redo = __ballot_sync(0xffffffffu, odd && live);
+      if (redo != 0) __syncwarp();            // other lanes stored pieces of these rows: their stores come first
       while (redo != 0) {
         const int rr = warp * 32 + __ffs(redo) - 1;
         redo &= redo - 1;

@@ -189,6 +189,18 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(cuda_devic
 
 
 @pytest.mark.parametrize("layout", ["plain", "odd"])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 128), (8, 2, 64), (16, 1, 128)])
+def test_whole_tiles_beside_a_masked_value_that_is_not_finite(cuda_device, layout, hq, hkv, d):
+    """Only the last key is NaN: all rows of its tiles but the last are formed again, in the place where
+    their first results were stored, also as split results."""
+    def edit(q, k, v):
+        v[-1] = float("nan")
+        return q, k, v
+    run([300], [0], hq, hkv, d, BF, edit=edit, layout=layout)
+    run([40], [3000], hq, hkv, d, FP, edit=edit, layout=layout)
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
 def test_rows_behind_the_last_sequence_stay(cuda_device, layout):
     q, k, v = (torch.randn(300, h, 128, device="cuda").to(BF) for h in (8, 2, 2))
     for t in (q, k, v):
