@@ -109,8 +109,9 @@ __device__ __forceinline__ int tiles_from(const SequenceSizes& z, int seqs, int 
 }
 
 // Sequence and tile of tile number `tile` (whole warp; every lane gets them); false past the last.
-// `chunk` and `before` are a cursor of the unsorted order: pass 0, 0 first and tiles in ascending
-// order.
+// `chunk` and `before` are a cursor of the unsorted order: pass 0, 0 first.  Tiles may come in any order,
+// as the hardware may hand out waiting blocks in any: ascending ones go on from the cursor, one that
+// lies before it starts over.
 __device__ __forceinline__ bool find_tile(const AttendLaunch& a, int step, int64_t tile, int& chunk, int64_t& before,
                                           int& q0, int& q1, int& k0, int& k1, int& index) {
   const int lane = threadIdx.x & 31;
@@ -178,6 +179,7 @@ __device__ __forceinline__ bool find_tile(const AttendLaunch& a, int step, int64
     }
     return false;
   }
+  if (tile < before) chunk = 0, before = 0;
   while (chunk < a.seqs) {
     const int s = chunk + lane;
     int n = 0;
