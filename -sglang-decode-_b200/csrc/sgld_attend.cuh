@@ -135,7 +135,7 @@ __device__ __forceinline__ bool find_tile(const AttendLaunch& a, int step, int64
   if (a.seqs <= kSortedSeqs) {
     // Level n holds the tiles of n blocks of 128 keys: the highest level whose tiles and all above
     // are more than `tile`, then the place within it, sequence by sequence.
-    const int most = a.window_left >= 0 ? a.window_left + step : 0x7fffffff;
+    const int most = a.window_left >= 0 ? min(a.window_left, 0x3fffffff) + step : 0x7fffffff;
     SequenceSizes z;
     int top = 0;
 #pragma unroll

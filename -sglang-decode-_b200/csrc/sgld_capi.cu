@@ -666,7 +666,9 @@ int prompt_launch(const sgld_prompt_args* args, sgld::AttendLaunch& a, bool& tc)
   a.page_size = 1;
   a.dtype = p.dtype;
   a.causal = 1;
-  a.window_left = p.window_left;
+  // A window that no key of the call can leave is none: the kernels subtract it from key positions in 32 bits,
+  // and those of queries before key 0 are negative.
+  a.window_left = p.window_left < a.kv_count ? p.window_left : -1;
   a.scale = p.scale;
   a.logit_cap = p.logit_cap;
   tc = prepare_attend(a);

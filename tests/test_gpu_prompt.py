@@ -1,4 +1,5 @@
 """Prompt attention on the GPU against the formula in 64 bits (tolerance: tests/attention_reference.py)."""
+import ctypes
 import random
 
 import pytest
@@ -86,6 +87,31 @@ def test_layouts(cuda_device, layout):
 @pytest.mark.parametrize("window", [0, 1, 63, 128, 500])
 def test_windows(cuda_device, window, layout):
     run([400, 1, 700], [0, 900, 130], 8, 2, 64, FP, pool=True, window=window, layout=layout)
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
+@pytest.mark.parametrize("window", [0, 39, 40, 41, 170, 2 ** 30, 2 ** 31 - 2, 2 ** 31 - 1])
+def test_windows_through_the_c_abi(cuda_device, window, layout):
+    """Any int32 window, 2^31 - 1 as "none" among them, with tiles whose first queries lie before key 0."""
+    q_lens, kv_lens = [100, 7], [41, 129]
+    q, k, v = (torch.randn(n, h, 128, device="cuda").to(BF) for n, h in ((107, 8), (170, 2), (170, 2)))
+    want = prompt(q, k, v, q_lens, kv_lens, window=window)
+    if layout == "odd":
+        q, k, v = odd_rows(q), odd_rows(k), odd_rows(v)
+    out, lse = torch.full((107, 8, 128), 5.0, device="cuda", dtype=BF), torch.zeros(107, 8, device="cuda")
+    q_indptr, kv_indptr = pointers(q_lens), pointers(kv_lens)
+    a = _native.PromptArgs()
+    a.q, a.k, a.v, a.out, a.lse = (x.data_ptr() for x in (q, k, v, out, lse))
+    a.q_indptr, a.kv_indptr = q_indptr.data_ptr(), kv_indptr.data_ptr()
+    for name, x in (("q", q), ("k", k), ("v", v), ("out", out)):
+        getattr(a, name + "_stride")[:] = x.stride()
+    a.kv_extent, a.tokens, a.seqs, a.query_heads, a.kv_heads, a.head_dim, a.dtype = 170, 107, 2, 8, 2, 128, 1
+    a.window_left, a.scale = window, 128 ** -0.5
+    size = _native.load().sgld_prompt_workspace_bytes(ctypes.byref(a))
+    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _native.load().sgld_prompt_attention(ctypes.byref(a), workspace.data_ptr(), size, stream) == 0
+    check(out, want, BF, 129, lse)
 
 
 @pytest.mark.parametrize("layout", ["plain", "odd"])
