@@ -236,8 +236,8 @@ cudaError_t launch_dim(const AttendLaunch& a, cudaStream_t stream) {
 // ---------------------------------------------------------------- merge of split results
 // One warp per (row, query head): the LSE-weighted sum of the row's split results, all of `second` (the
 // prefix, or a prompt's splits) and then `first` (a decode's counts[row] slots of first_max; absent
-// for the prompt attention), each in split order.  A slot whose LSE is -inf saw no key: its values
-// do not count.  A row is a chain of two memory round trips (its count, its slots), which bound the
+// for the prompt attention, and for a decode without an index of own tokens, whose rows with counts
+// are NaN), each in split order.  A slot whose LSE is -inf saw no key: its values do not count.  A row is a chain of two memory round trips (its count, its slots), which bound the
 // kernel, not the bytes: values are loaded together with their LSEs, four slots at a time, at 64
 // registers for 32 warps an SM (16384 rows of 3 slots: 23 us; with eight slots and their values only
 // after the LSEs, at 96 registers, 34).
@@ -252,6 +252,7 @@ struct MergeLaunch {
   void* out;
   float* lse;
   int32_t* claim;
+  int32_t* status;           // bit 512: a row has own tokens but no index names them
   int64_t out_stride[3];
   int32_t first_max, second_max, rows, rows_second, heads, head_dim;
   const int32_t* q_indptr;   // rows at or past q_indptr[seqs] are left as they are
@@ -305,7 +306,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 8) merge_shared_kernel(const
   if (a.q_indptr != nullptr && (row < a.q_indptr[0] || row >= a.q_indptr[a.seqs])) return;
   const bool err = a.error != nullptr && *a.error != 0;
   const bool shared = row < a.rows_second && (a.active == nullptr || row < *a.active);
-  const int n = a.first != nullptr ? a.counts[row] : 0;
+  int n = a.counts != nullptr ? a.counts[row] : 0;
+  const bool lost = n > 0 && a.first == nullptr;
+  if (lost) {
+    if (head == 0 && lane == 0) atomicOr(a.status, 512);
+    n = 0;
+  }
   for (int d = lane * 4; d < a.head_dim; d += 128) {
     Running r{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
     if (shared)
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, 8) merge_shared_kernel(const
     const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
     float v[4] = {r.acc.x * inv, r.acc.y * inv, r.acc.z * inv, r.acc.w * inv};
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.out_stride[0] + static_cast<int64_t>(head) * a.out_stride[1];
-    if (err) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
+    if (err || lost) v[0] = v[1] = v[2] = v[3] = __int_as_float(0x7fc00000);
     if (a.out_stride[2] == 1 && (reinterpret_cast<uintptr_t>(out + d) & 7) == 0) {
       *reinterpret_cast<uint2*>(out + d) = make_uint2(Mma<T>::pack(v[0], v[1]), Mma<T>::pack(v[2], v[3]));
     } else {
@@ -366,7 +372,7 @@ cudaError_t launch_merge_prompt(const AttendLaunch& a, void* out, float* lse, cu
 cudaError_t launch_merge_prefix(const AttendLaunch& a, const sgld_decode_args& d, const sgld_plan_buffers& p, int bcap,
                                 int smax, cudaStream_t stream) {
   MergeLaunch m = {};
-  m.first = d.partial;
+  m.first = d.pages != nullptr ? d.partial : nullptr;
   m.first_lse = d.lse;
   m.counts = p.counts;
   m.first_max = smax;
@@ -377,6 +383,7 @@ cudaError_t launch_merge_prefix(const AttendLaunch& a, const sgld_decode_args& d
   m.active = p.active;
   m.out = d.out;
   m.claim = d.counter;
+  m.status = d.status;
   m.out_stride[0] = static_cast<int64_t>(d.query_heads) * d.head_dim;
   m.out_stride[1] = d.head_dim;
   m.out_stride[2] = 1;

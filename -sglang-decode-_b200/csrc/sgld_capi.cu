@@ -255,13 +255,13 @@ namespace sgld {
 // Every host-side check of sgld_decode_persistent, with nothing enqueued: shapes, dtypes,
 // pointers (scratch included), strides and capacities.  SGLD_OK when a launch may follow.
 int validate_decode(const sgld_decode_args* args, const sgld_plan_buffers* plan,
-                    const sgld_plan_geometry* geometry) {
+                    const sgld_plan_geometry* geometry, bool own_tokens) {
   if (args == nullptr) return fail(SGLD_ERR_INVALID_ARGUMENT, "decode args are NULL");
   int rc = check_geometry(geometry);
   if (rc) return rc;
   if ((rc = check_plan_pointers(plan))) return rc;
   const sgld_decode_args& d = *args;
-  if (!d.q || !d.k || !d.v || !d.out || !d.pages || !d.counter || !d.partial || !d.lse || !d.status)
+  if (!d.q || !d.k || !d.v || !d.out || (own_tokens && !d.pages) || !d.counter || !d.partial || !d.lse || !d.status)
     return fail(SGLD_ERR_INVALID_ARGUMENT, "a tensor or scratch pointer is NULL");
   if (!aligned16(d.partial))   // the epilogue and the merge move partial rows as float4
     return fail(SGLD_ERR_INVALID_ARGUMENT, "partial must be 16-byte aligned");
@@ -446,7 +446,8 @@ int run_decode(const sgld_decode_args& d, const sgld_plan_buffers* plan, const s
     e = prefix_tc ? sgld::launch_attend_tc(*prefix, st) : sgld::launch_attend_mma(*prefix, st);
     if (e != cudaSuccess) return cuda_fail(e, "sgld_decode_shared_prefix prefix launch");
   }
-  if (kind == SGLD_KERNEL_TCGEN05 || kind == SGLD_KERNEL_TCGEN05_TMA) e = sgld::launch_decode_tc(a, st);
+  if (prefix != nullptr && d.pages == nullptr) e = cudaSuccess;   // no own tokens: the prefix alone
+  else if (kind == SGLD_KERNEL_TCGEN05 || kind == SGLD_KERNEL_TCGEN05_TMA) e = sgld::launch_decode_tc(a, st);
   else if (kind == SGLD_KERNEL_SMALL) e = sgld::launch_decode_small(a, st);
   else e = sgld::launch_decode(a, st);
   if (e != cudaSuccess) return cuda_fail(e, "sgld_decode_persistent launch");
@@ -740,7 +741,7 @@ size_t sgld_prefix_workspace_bytes(int32_t batch_capacity, int32_t query_heads, 
 
 int sgld_decode_shared_prefix(const sgld_decode_args* args, const sgld_prefix_args* prefix,
                               const sgld_plan_buffers* plan, const sgld_plan_geometry* geometry, void* stream) {
-  const int rc = sgld::validate_decode(args, plan, geometry);
+  const int rc = sgld::validate_decode(args, plan, geometry, args != nullptr && args->pages != nullptr);
   if (rc) return rc;
   if (prefix == nullptr) return fail(SGLD_ERR_INVALID_ARGUMENT, "prefix args are NULL");
   const sgld_decode_args& d = *args;

@@ -82,9 +82,10 @@ cudaError_t launch_decode_tc(const DecodeLaunch& a, cudaStream_t stream);
 int set_last_error(int code, const char* msg);
 
 // Every host-side check of sgld_decode_persistent (nothing is enqueued); SGLD_OK or the
-// status that call would return, with sgld_last_error() set.
+// status that call would return, with sgld_last_error() set.  own_tokens: the call decodes own tokens, whose
+// index `pages` must then be given.
 int validate_decode(const sgld_decode_args* args, const sgld_plan_buffers* plan,
-                    const sgld_plan_geometry* geometry);
+                    const sgld_plan_geometry* geometry, bool own_tokens = true);
 
 // The calling thread's current CUDA context (a CUcontext), nullptr if unknown.
 void* current_context();

@@ -222,8 +222,7 @@ void decode_shared_prefix(const at::Tensor& q, const at::Tensor& k, const at::Te
   const sgld_plan_buffers p = plan_of(plan, g);
   sgld_decode_args a = decode_args(q, k, v, pages, indptr, out, partial, lse, counter, status, g, page_size, scale, logit_cap,
                                    1.0, 1.0, k_new, v_new, new_loc);
-  // No request has own tokens: an empty index tensor has no address, and none of it is read.
-  if (pages.numel() == 0) a.pages = p.lengths;
+  if (pages.numel() == 0) a.pages = nullptr;   // no request may have own tokens: nothing is read for them
   sgld_prefix_args x;
   std::memset(&x, 0, sizeof(x));
   x.index = prefix.size(0) > 0 ? prefix.data_ptr<int32_t>() : nullptr;

@@ -47,7 +47,8 @@ class SharedPrefixEngine(DecodeEngine):
         ``prefix_length`` (int32[1] on the GPU; default: all that ``prefix`` names) lets a captured
         call follow a prefix whose length changes; lengths past what ``prefix`` names are cut to it.
         An index outside the pool reads as a zero row.  Requests without own tokens attend to the
-        prefix alone; rows at or past the plan's active count are zero.  K/V have Q's dtype (no
+        prefix alone; rows at or past the plan's active count are zero.  With CSR KV ``pages`` may be
+        empty where no request has own tokens (one that has some gets a NaN row and sets status 512).  K/V have Q's dtype (no
         fp8), and a paged pool's pages lie one after another.  ``scale`` must be > 0.  The call can
         be captured (``DecodeGraph`` itself captures plain engines only).
         """
@@ -64,7 +65,9 @@ class SharedPrefixEngine(DecodeEngine):
         return out.output
 
     def kernel_kind(self, layer=0):
-        """Name of the decode kernel of the own tokens; the small-batch kernel, which merges the
-        splits itself, is never among them."""
+        """Name of the decode kernel of the own tokens ("none" for empty ``pages``); the small-batch kernel,
+        which merges the splits itself, is never among them."""
+        if self._calls[layer][3].numel() == 0:
+            return "none"
         kind = super().kernel_kind(layer)
         return "mma.sync" if kind == "small" else kind

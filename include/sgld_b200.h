@@ -155,7 +155,8 @@ typedef struct sgld_decode_args {
   float* partial;       /* [B, Hq, Smax, D] fp32 normalised split outputs, 16-byte aligned   */
   float* lse;           /* [B, Hq, Smax]    fp32 natural-log LSE per split                   */
   int32_t* status;      /* [1]  0 = ok; otherwise sticky error bits: 1-32 a bounded in-kernel
-                           wait expired, 64 q_rows too small, 128 a new_loc slot out of range */
+                           wait expired, 64 q_rows too small, 128 a new_loc slot out of range,
+                           512 own tokens without an index (sgld_decode_shared_prefix)      */
 } sgld_decode_args;
 
 /*
@@ -327,7 +328,8 @@ int sgld_prompt_kernel_kind(const sgld_prompt_args* args);
  * sgld_decode_persistent).  The prefix's K and V are read once for all requests, whose query rows
  * form the rows of one matrix product; the decode of the own tokens follows, and one merge
  * combines both.  Requests without own tokens get the prefix alone; rows past the plan's active
- * count are zero.  K/V of `dtype` (fp8 pools: SGLD_ERR_UNSUPPORTED); a paged pool must have its
+ * count are zero.  args->pages may be NULL where no request has own tokens: their decode is then left
+ * out, and a request that has some all the same gets a NaN row and sets status bit 512.  K/V of `dtype` (fp8 pools: SGLD_ERR_UNSUPPORTED); a paged pool must have its
  * pages one after another (k_stride[0] == page_size * k_stride[1], v likewise).
  */
 typedef struct sgld_prefix_args {

@@ -171,6 +171,22 @@ def test_an_inactive_row_and_a_broken_plan(cuda_device):
     assert s.run().isnan().all()
 
 
+def test_no_index_of_own_tokens(cuda_device):
+    """Empty ``pages``: the prefix alone, and a NaN row where the plan gives a request own tokens."""
+    s = Setup([0, 0, 0], 300, 8, 2, 128, BF)
+    assert s.pages.numel() == 0
+    s.check(s.run())
+    assert s.engine.kernel_kind() == "none"
+    s.engine.plan.lengths[1] = 1            # (the capacity: more is a broken plan)
+    out = s.run().clone()
+    assert out[1].isnan().all() and s.engine.layers[0].status.item() == 512
+    check(out[::2], [x[::2] for x in s.want()], BF, 300)
+    assert s.engine.layers[0].counter.tolist() == [0, 0]
+    s.engine.plan.lengths[1] = 0
+    s.engine.layers[0].status.zero_()
+    s.check(s.run())
+
+
 def test_smaller_prefix_than_the_capacity_and_layers(cuda_device):
     s = Setup([9, 30], 640, 32, 8, 128, BF, prefix_capacity=20000)
     s.check(s.run())
