@@ -48,7 +48,7 @@ __device__ __forceinline__ void copy_chunk(T* dst, const T* src, int64_t stride,
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attend_mma_kernel(const __grid_constant__ AttendLaunch a) {
+__global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attend_mma_kernel(const __grid_constant__ AttendLaunch a) {
   constexpr int kB = key_block<D>(), kP = pitch<D>(), kNb = kB / 8, kDb = D / 8;
   constexpr float kBias = WeightBias<T>::value;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) attend_mma_kernel(const __grid_const
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     const int r = warp * 16 + lane / 4 + 8 * h, row = t.first + r / G, head = t.head * G + r % G;
     const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
-    const float e = l[h] == 0.f ? -INFINITY : (m[h] - kBias + lg2(l[h])) * kLn2;
+    const float e2 = l[h] == 0.f ? -INFINITY : m[h] - kBias + lg2(l[h]);
     const int64_t at = static_cast<int64_t>(row) * a.query_heads + head;
     bool odd = false;
     if (r < rows) {
@@ -191,18 +191,13 @@ __global__ void __launch_bounds__(kThreads) attend_mma_kernel(const __grid_const
         }
       }
       if ((lane & 3) == 0) {
-        if (a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = e;
-        else if (a.lse != nullptr) a.lse[at] = e;
+        if (a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = e2 * kLn2;
+        else if (a.lse != nullptr) a.lse[at] = e2 * kLn2;
       }
     }
-    uint32_t redo = __ballot_sync(0xffffffffu, odd);
-    __syncwarp();
-    while (redo != 0) {                       // one lane of each such row, then its whole warp
-      const int who = __ffs(redo) - 1;
-      redo &= ~(0xfu << (who & ~3));
-      const int rr = warp * 16 + who / 4 + 8 * h;
-      redo_row<T>(a, t, t.first + rr / G, t.head * G + rr % G, 0, D);
-    }
+    uint32_t again = __ballot_sync(0xffffffffu, odd);
+    again = __ballot_sync(0xffffffffu, (lane & 3) == 0 && (again >> lane & 0xfu) != 0);   // one lane of each such row
+    if (again != 0) form_again<T, D>(a, t, again, row, head, e2, nullptr);
   }
 }
 

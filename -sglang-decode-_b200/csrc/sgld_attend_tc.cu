@@ -74,20 +74,44 @@ struct Misc {
   alignas(16) uint64_t claim[2];
   AttendTask task[kTaskRing];
   uint32_t tmem_base;
+  uint64_t beat;               // time of form_again's last step: waits behind it go on
 };
 static_assert(sizeof(Misc) <= 1024, "misc area too small");
 static_assert(Layout<128>::kBytes <= 232448 && Layout<64>::kBytes <= 232448, "shared memory budget exceeded");
 
 enum : int { kStatusWait = 1 };
 
-__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity) {
-  return mbar_wait(bar, parity, global_timer_ns() + kWaitLimitNs);
+// A wait expires when 4 s have passed since it began and since the last step of form_again in this CTA: with
+// bad values in a long sequence those steps can take longer, and end by themselves.  One block of
+// assembly: as C++ the compiler lays the loop out between the instructions of the roles' own loops, and
+// the kernel is 3 to 12% slower for it (the forms differed, the work did not).
+__device__ __forceinline__ bool bounded_wait(Misc& ms, uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 start, now, beat;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "mov.u64 start, %%globaltimer;\n\t"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "ld.volatile.shared::cta.u64 beat, [%3];\n\t"
+      "mov.u64 now, %%globaltimer;\n\t"
+      "max.u64 beat, beat, start;\n\t"
+      "sub.u64 now, now, beat;\n\t"
+      "setp.lt.u64 q, now, %4;\n\t"
+      "@q bra AGAIN;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(&ms.beat)), "n"(kWaitLimitNs)
+      : "memory");
+  return ok != 0;
 }
 
 // Bounded wait of a whole warp, which it reconverges.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
-  bool ok = mbar_try_wait(bar, parity) || wait_slow(bar, parity);
-  ok = __all_sync(0xffffffffu, ok);
+__device__ __forceinline__ bool warp_wait(Misc& ms, uint64_t* bar, uint32_t parity, int* status) {
+  const bool ok = __all_sync(0xffffffffu, bounded_wait(ms, bar, parity));
   if (!ok && status != nullptr && (threadIdx.x & 31) == 0) atomicOr(status, kStatusWait);
   return ok;
 }
@@ -220,7 +244,7 @@ struct Attend {
   }
   // The answer: the block's number, or -1 when none is left.
   __device__ static bool next_task(Misc& ms, int& asked, uint32_t& phase, int64_t& task, int* status) {
-    if (!warp_wait(&ms.claimed, phase, status)) return false;
+    if (!warp_wait(ms, &ms.claimed, phase, status)) return false;
     --asked;
     phase ^= 1u;
     const volatile uint64_t* r = ms.claim;
@@ -260,13 +284,13 @@ struct Attend {
           claim_task(ms, asked);
           if (!next_task(ms, asked, cph, task, status)) return;
         }
-        if (!warp_wait(&ms.tempty[tr.i], tr.phase ^ 1u, status)) return;
+        if (!warp_wait(ms, &ms.tempty[tr.i], tr.phase ^ 1u, status)) return;
         if (lane == 0) {
           ms.task[tr.i] = t;
           mbar_arrive(&ms.tfull[tr.i]);
         }
       } else {
-        if (!warp_wait(&ms.tfull[tr.i], tr.phase, status)) return;
+        if (!warp_wait(ms, &ms.tfull[tr.i], tr.phase, status)) return;
         t = ms.task[tr.i];
         __syncwarp();
         if (lane == 0) mbar_arrive(&ms.tempty[tr.i]);
@@ -289,7 +313,7 @@ struct Attend {
         if (b == blocks - 1 && w == 0) claim_task(ms, asked);      // late: the SM that is done first takes the next
         if (b + 1 < blocks) look_up(a, t, w, t.lo + (b + 1) * kRows, next, next_boxes);   // in flight during the waits
         if (b == 0 && w == 0) {                             // Q right before the first K
-          if (!warp_wait(&ms.q_empty, qph ^ 1u, status)) return;
+          if (!warp_wait(ms, &ms.q_empty, qph ^ 1u, status)) return;
           qph ^= 1u;
           if (lane == 0) {
             const int tiles = t.first + tokens < t.last ? 2 : 1;
@@ -304,7 +328,7 @@ struct Attend {
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {                       // K, then V
-          if (!warp_wait(&ms.kv_empty[kv.i], kv.phase ^ 1u, status)) return;
+          if (!warp_wait(ms, &ms.kv_empty[kv.i], kv.phase ^ 1u, status)) return;
           ++issued;
           const uint32_t dst = smem_addr(smem + L::kOffRing + kv.i * L::kTile);
           if (boxes > 0) {
@@ -342,13 +366,13 @@ struct Attend {
     int asked = 0;
     uint32_t cph = 0;
     load_tasks(a, smem, ms, w, issued, q_issued, asked, cph);
-    if (asked > 0) warp_wait(&ms.claimed, cph, a.status);
+    if (asked > 0) warp_wait(ms, &ms.claimed, cph, a.status);
     asm volatile("cp.async.wait_all;" ::: "memory");
     for (int i = 0; i < L::kStages && i < issued; ++i) {
       const int64_t last = issued - 1 - (issued - 1 - i) % L::kStages;      // the last tile put into stage i
-      warp_wait(&ms.kv_full[i], static_cast<uint32_t>(last / L::kStages) & 1u, a.status);
+      warp_wait(ms, &ms.kv_full[i], static_cast<uint32_t>(last / L::kStages) & 1u, a.status);
     }
-    if (q_issued > 0) warp_wait(&ms.q_full, static_cast<uint32_t>(q_issued - 1) & 1u, a.status);
+    if (q_issued > 0) warp_wait(ms, &ms.q_full, static_cast<uint32_t>(q_issued - 1) & 1u, a.status);
   }
 
   // ------------------------------------------------------------------ MMA issuer (1 warp)
@@ -402,7 +426,7 @@ struct Attend {
     mma_tasks(a, smem, ms);
     __syncwarp();
     commit(&ms.drain);
-    warp_wait(&ms.drain, 0, a.status);
+    warp_wait(ms, &ms.drain, 0, a.status);
   }
 
   __device__ static void mma_tasks(const AttendLaunch& a, unsigned char* smem, Misc& ms) {
@@ -415,7 +439,7 @@ struct Attend {
     Ring kv, tr;
     uint32_t qph = 0, pph[2] = {0, 0}, oph[2] = {1, 1};
     while (true) {
-      if (!warp_wait(&ms.tfull[tr.i], tr.phase, status)) return;
+      if (!warp_wait(ms, &ms.tfull[tr.i], tr.phase, status)) return;
       const AttendTask t = ms.task[tr.i];
       __syncwarp();
       if (lane == 0) mbar_arrive(&ms.tempty[tr.i]);
@@ -427,7 +451,7 @@ struct Attend {
       n[1] = __shfl_sync(0xffffffffu, n[1], 0);
       const int blocks = max(n[0], n[1]);
       if (blocks == 0) continue;
-      if (!warp_wait(&ms.q_full, qph, status) || !warp_wait(&ms.kv_full[kv.i], kv.phase, status)) return;
+      if (!warp_wait(ms, &ms.q_full, qph, status) || !warp_wait(ms, &ms.kv_full[kv.i], kv.phase, status)) return;
       qph ^= 1u;
       fence_proxy_async_smem();               // row copies arrive through the generic proxy
       tc_fence_after();
@@ -444,19 +468,19 @@ struct Attend {
       for (int b = 0; b < blocks; ++b) {
         const Ring v = kv;                    // V of this block, then K of the next
         kv.next(L::kStages);
-        if (!warp_wait(&ms.kv_full[v.i], v.phase, status)) return;
-        if (b + 1 < blocks && !warp_wait(&ms.kv_full[kv.i], kv.phase, status)) return;
+        if (!warp_wait(ms, &ms.kv_full[v.i], v.phase, status)) return;
+        if (b + 1 < blocks && !warp_wait(ms, &ms.kv_full[kv.i], kv.phase, status)) return;
         fence_proxy_async_smem();
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if (b < n[g]) {
             if (b == 0) {
-              if (!warp_wait(&ms.o_free[g], oph[g], status)) return;
+              if (!warp_wait(ms, &ms.o_free[g], oph[g], status)) return;
               oph[g] ^= 1u;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (!warp_wait(&ms.p_ready[g][h], pph[g], status)) return;
+              if (!warp_wait(ms, &ms.p_ready[g][h], pph[g], status)) return;
               tc_fence_after();
               issue_pv(vdesc + v.i * (L::kTile >> 4), g, h, b == 0 ? 1u : 0u);
             }
@@ -689,7 +713,7 @@ struct Attend {
     uint32_t sph = 0, oph = 0;
     bool ok = true;
     while (ok) {
-      if (!warp_wait(&ms.tfull[tr.i], tr.phase, status)) return;
+      if (!warp_wait(ms, &ms.tfull[tr.i], tr.phase, status)) return;
       const AttendTask t = ms.task[tr.i];
       __syncwarp();
       if (lane == 0) mbar_arrive(&ms.tempty[tr.i]);
@@ -704,7 +728,7 @@ struct Attend {
       const int lo = live ? first_key(a, t, row) : 0, hi = live ? last_key(a, t, row) : 0x3fffffff;
       float m = -INFINITY, l = 0.f;
       for (int b = 0; b < blocks; ++b) {
-        ok = warp_wait(&ms.s_full[g], sph, status);
+        ok = warp_wait(ms, &ms.s_full[g], sph, status);
         if (!ok) break;
         sph ^= 1u;
         tc_fence_after();
@@ -732,11 +756,12 @@ struct Attend {
       }
       const int64_t at = static_cast<int64_t>(row) * a.query_heads + head;
       if (blocks > 0 && ok) {
-        ok = warp_wait(&ms.o_full[g], oph, status);
+        ok = warp_wait(ms, &ms.o_full[g], oph, status);
         oph ^= 1u;
         tc_fence_after();
       }
       const float inv = !ok ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.f / l;
+      const float e2 = l == 0.f ? -INFINITY : m - kBias + lg2(l);
       bool odd = false;
       unsigned char* dst = nullptr;
       if (live)
@@ -772,19 +797,14 @@ struct Attend {
         }
         odd = !(check == 0.f);
         if (live) {
-          const float e = !ok ? inv : l == 0.f ? -INFINITY : (m - kBias + lg2(l)) * kLn2;
+          const float e = !ok ? inv : e2 * kLn2;
           if (a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = e;
           else if (a.lse != nullptr) a.lse[at] = e;
         }
       }
       if (!ok) return;
-      uint32_t redo = __ballot_sync(0xffffffffu, odd && live);
-      if (redo != 0) __syncwarp();            // other lanes stored pieces of these rows: their stores come first
-      while (redo != 0) {
-        const int rr = warp * 32 + __ffs(redo) - 1;
-        redo &= redo - 1;
-        redo_row<T>(a, t, t.first + g * tokens + rr / G, t.head * G + rr % G, 0, D);
-      }
+      const uint32_t again = __ballot_sync(0xffffffffu, odd && live);
+      if (again != 0) form_again<T, D>(a, t, again, row, head, e2, &ms.beat);
     }
   }
 };
@@ -798,6 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   Misc& ms = *reinterpret_cast<Misc*>(smem + L::kOffMisc);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
+    ms.beat = 0;
     for (int i = 0; i < L::kStages; ++i) mbar_init(&ms.kv_full[i], kLoaders * 32), mbar_init(&ms.kv_empty[i], 1);
     mbar_init(&ms.q_full, 1), mbar_init(&ms.q_empty, 1), mbar_init(&ms.drain, 1), mbar_init(&ms.claimed, 1);
     for (int g = 0; g < 2; ++g)

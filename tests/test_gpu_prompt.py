@@ -226,6 +226,75 @@ def test_whole_tiles_beside_a_masked_value_that_is_not_finite(cuda_device, layou
     run([40], [3000], hq, hkv, d, FP, edit=edit, layout=layout)
 
 
+BAD = {
+    "one early key": lambda v: v[5, :, 3].fill_(float("nan")),
+    "all from the middle on": lambda v: v[v.shape[0] // 2:].fill_(float("nan")),
+    "an infinity in every 64 keys": lambda v: v[::64, :, 7].fill_(float("inf")),
+    "both infinities and a NaN, dims apart": lambda v: (v[70, :, 0].fill_(float("inf")), v[90, :, 0].fill_(-float("inf")),
+                                                        v[90, :, 1].fill_(-float("inf")), v[131, :, 1].fill_(float("nan")),
+                                                        v[-1, :, 2].fill_(float("inf"))),
+    "the last keys": lambda v: v[-3:].fill_(-float("inf")),
+}
+
+
+@pytest.mark.parametrize("d,layout", [(128, "plain"), (64, "plain"), (64, "odd"), (128, "odd"), (256, "plain")])
+@pytest.mark.parametrize("bad", list(BAD))
+def test_what_a_row_becomes_beside_values_that_are_not_finite(cuda_device, bad, d, layout):
+    """Rows that see them, in the dims that have them, and no others; causal, on cache slots, in a window
+    whose lower edge passes them, and as split results."""
+    def edit(q, k, v):
+        v = v.clone()
+        BAD[bad](v)
+        return q, k, v
+    run([333], [0], 8, 2, d, BF, edit=edit, layout=layout)
+    run([150, 40], [300, 0], 4, 4, d, FP, edit=edit, layout=layout, pool=True, cap=15.0)
+    run([333], [100], 16, 1, d, BF, edit=edit, layout=layout, window=70)
+    run([3], [1500], 8, 2, d, FP, edit=edit, layout=layout)
+
+
+@pytest.mark.parametrize("layout", ["plain", "odd"])
+def test_sums_that_pass_the_largest_number_on_the_way(cuda_device, layout):
+    """Values of 2^124 under equal weights: their weighted sum before the division does not fit fp32."""
+    q, k = (torch.zeros(300, h, 128, device="cuda", dtype=BF) for h in (4, 4))
+    v = torch.full((300, 4, 128), 2.0 ** 124, device="cuda", dtype=BF)
+    if layout == "odd":
+        q, k, v = odd_rows(q), odd_rows(k), odd_rows(v)
+    out = prompt_attention(q, k, v, pointers([300]))
+    check(out, prompt(q, k, v, [300], [300]), BF, 300)
+
+
+@pytest.mark.parametrize("bad", ["one early key", "all from the middle on", "an infinity in every 64 keys", "K"])
+def test_bad_values_in_a_long_prompt_cost_no_second_pass_for_each_row(cuda_device, bad):
+    """4096 tokens of 16 heads.  A walk of every row over its own keys would be 1.3e8 dependent steps of
+    1.7 us (measured so at 1024 tokens) by 1184 warps, 190 ms; whole warps search 2048 tiles of at most
+    4096 keys.  The best of three runs is bounded by a fifth of the walk."""
+    q, k, v = (torch.randn(4096, h, 128, device="cuda").to(BF) for h in (16, 4, 4))
+    if bad == "K":
+        k[5] = float("nan")
+    else:
+        BAD[bad](v)
+    status, ends = torch.zeros(1, dtype=torch.int32, device="cuda"), pointers([4096])
+    out = prompt_attention(q, k, v, ends, status=status)
+    times = []
+    for _ in range(3):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        prompt_attention(q, k, v, ends, out=out, status=status)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    assert min(times) < 38 and status.item() == 0
+    some = torch.tensor([0, 4, 5, 6, 63, 64, 65, 1000, 2047, 2048, 2049, 4095], device="cuda")
+    finite = torch.isfinite(out[some])
+    rows = some[:, None]
+    seen = {"K": rows >= 5, "one early key": rows >= 5, "all from the middle on": rows >= 2048,
+            "an infinity in every 64 keys": rows >= 0}[bad][:, None].expand(-1, 16, 128).clone()
+    if bad not in ("K", "all from the middle on"):
+        dim = 3 if bad == "one early key" else 7
+        seen[..., :dim] = seen[..., dim + 1:] = False
+    assert torch.equal(finite, ~seen)
+
+
 @pytest.mark.parametrize("layout", ["plain", "odd"])
 def test_rows_behind_the_last_sequence_stay(cuda_device, layout):
     q, k, v = (torch.randn(300, h, 128, device="cuda").to(BF) for h in (8, 2, 2))
