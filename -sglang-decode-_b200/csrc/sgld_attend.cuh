@@ -54,6 +54,8 @@ struct alignas(64) AttendLaunch {
                                // page, 0 where every row is copied by itself
   int32_t aligned;             // every row 16-byte aligned with unit stride along D
   float scale, logit_cap;
+  int32_t stall;               // tasks after which the tcgen05 kernel's issuer stops in every CTA (tests); -1: never
+  uint64_t wait_ns;            // after which its waits expire
 };
 
 cudaError_t launch_attend_mma(const AttendLaunch& a, cudaStream_t stream);

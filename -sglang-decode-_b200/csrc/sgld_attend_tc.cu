@@ -28,8 +28,9 @@
 // Precision: scores, maxima, sums and O are fp32; p is rounded to 16 bits for the second product
 // (its operand type), the sum keeps the fp32 values.
 //
-// Every wait is bounded (4 s); a role whose wait expires sets a status bit and leaves, the
-// softmax with NaN rows, and tensor memory is freed on every path.
+// Every wait is bounded (4 s); a role whose wait expires sets a status bit and makes the others' waits
+// expire, the copies and MMAs in flight are awaited, the rows of all tasks that the CTA had taken and
+// may not have stored are set to NaN (give_up), and tensor memory is freed on every path.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -43,13 +44,18 @@
 namespace sgld {
 namespace {
 
-constexpr uint64_t kWaitLimitNs = 4000000000ull;
+constexpr uint64_t kDrainLimitNs = 4000000000ull;   // of the waits for a CTA's own copies and MMAs at its end
+constexpr uint64_t kFailed = ~0ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kRows = 128;                 // rows of a tile (MMA M) and keys of a block (MMA N)
 constexpr int kMmaWarp = 0, kLoaderWarp = 1, kLoaders = 3, kSoftmaxWarp = 4, kWarps = 12, kThreads = kWarps * 32;
 constexpr int kTaskRing = 4;
+// Tasks that a CTA has taken and may not have stored: the one that the slowest softmax warp is at, the ring's,
+// one found and not published, one claimed.
+constexpr int kTaken = 8;
+static_assert(kTaken >= kTaskRing + 3, "tasks not stored are among the last taken");
 constexpr int kTmemCols = 512;             // S at 0 and 128 (P over S), O at 256 and 256 + D
 constexpr uint32_t kTmem = 0;              // all of tensor memory is allocated: it starts at column 0
 // Registers a thread: 384 x 168 at launch; the softmax groups take 208, the others keep 88.
@@ -64,6 +70,12 @@ struct Layout {
   static constexpr int kBytes = kOffMisc + 1024 + 1024;  // misc, and slack to align the base to 1 KB
 };
 
+// What a wait looks at once it does not succeed at once.
+struct alignas(16) Clock {
+  uint64_t beat;               // time of form_again's last step: waits behind it go on; kFailed: all expire
+  uint64_t limit;              // ns since `beat` and since the wait began
+};
+
 struct Misc {
   uint64_t kv_full[10], kv_empty[10];
   uint64_t q_full, q_empty;
@@ -74,44 +86,57 @@ struct Misc {
   alignas(16) uint64_t claim[2];
   AttendTask task[kTaskRing];
   uint32_t tmem_base;
-  uint64_t beat;               // time of form_again's last step: waits behind it go on
+  Clock clock, drain_clock;
+  int64_t issued[kLoaders];    // ring tiles that each loader has arrived for, at its end
+  uint32_t taken[kTaken], n_taken, lost;   // the last tasks taken; lost: a claim without an answer
 };
 static_assert(sizeof(Misc) <= 1024, "misc area too small");
 static_assert(Layout<128>::kBytes <= 232448 && Layout<64>::kBytes <= 232448, "shared memory budget exceeded");
 
 enum : int { kStatusWait = 1 };
 
-// A wait expires when 4 s have passed since it began and since the last step of form_again in this CTA: with
-// bad values in a long sequence those steps can take longer, and end by themselves.  One block of
-// assembly: as C++ the compiler lays the loop out between the instructions of the roles' own loops, and
-// the kernel is 3 to 12% slower for it (the forms differed, the work did not).
-__device__ __forceinline__ bool bounded_wait(Misc& ms, uint64_t* bar, uint32_t parity) {
+// A wait expires when clock.limit has passed since it began and since the last step of form_again in this
+// CTA (with bad values in a long sequence those steps can take longer, and end by themselves), or when
+// another has expired.  One block of assembly: as C++ the compiler lays the loop out between the
+// instructions of the roles' own loops, and the kernel is 3 to 12% slower for it (the forms differed,
+// the work did not).
+__device__ __forceinline__ bool bounded_wait(const Clock& clock, uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 start, now, beat;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 start, now, beat, limit;\n\t"
       "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra DONE;\n\t"
       "mov.u64 start, %%globaltimer;\n\t"
       "AGAIN:\n\t"
       "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
       "@p bra DONE;\n\t"
-      "ld.volatile.shared::cta.u64 beat, [%3];\n\t"
+      "ld.volatile.shared::cta.v2.u64 {beat, limit}, [%3];\n\t"
       "mov.u64 now, %%globaltimer;\n\t"
-      "max.u64 beat, beat, start;\n\t"
+      "max.u64 beat, beat, start;\n\t"          // kFailed: now - beat wraps to now + 1
       "sub.u64 now, now, beat;\n\t"
-      "setp.lt.u64 q, now, %4;\n\t"
+      "setp.lt.u64 q, now, limit;\n\t"
       "@q bra AGAIN;\n\t"
       "DONE:\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(&ms.beat)), "n"(kWaitLimitNs)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(smem_addr(&clock))
       : "memory");
   return ok != 0;
 }
 
 // Bounded wait of a whole warp, which it reconverges.
 __device__ __forceinline__ bool warp_wait(Misc& ms, uint64_t* bar, uint32_t parity, int* status) {
-  const bool ok = __all_sync(0xffffffffu, bounded_wait(ms, bar, parity));
+  const bool ok = __all_sync(0xffffffffu, bounded_wait(ms.clock, bar, parity));
+  if (!ok && (threadIdx.x & 31) == 0) {
+    atomicMax(reinterpret_cast<unsigned long long*>(&ms.clock.beat), static_cast<unsigned long long>(kFailed));
+    if (status != nullptr) atomicOr(status, kStatusWait);
+  }
+  return ok;
+}
+
+// The same at a role's end, for what the CTA itself has in flight, also after a failure.
+__device__ __forceinline__ bool drain_wait(Misc& ms, uint64_t* bar, uint32_t parity, int* status) {
+  const bool ok = __all_sync(0xffffffffu, bounded_wait(ms.drain_clock, bar, parity));
   if (!ok && status != nullptr && (threadIdx.x & 31) == 0) atomicOr(status, kStatusWait);
   return ok;
 }
@@ -243,10 +268,7 @@ struct Attend {
     __syncwarp();
   }
   // The answer: the block's number, or -1 when none is left.
-  __device__ static bool next_task(Misc& ms, int& asked, uint32_t& phase, int64_t& task, int* status) {
-    if (!warp_wait(ms, &ms.claimed, phase, status)) return false;
-    --asked;
-    phase ^= 1u;
+  __device__ static int64_t answer(Misc& ms) {
     const volatile uint64_t* r = ms.claim;
     const uint64_t lo = r[0], hi = r[1];
     uint32_t given, x;
@@ -256,9 +278,18 @@ struct Attend {
         "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, c;\n\t}"
         : "=r"(given), "=r"(x)
         : "l"(lo), "l"(hi));
-    task = given != 0 ? static_cast<int64_t>(x) : -1;
     __syncwarp();
+    return given != 0 ? static_cast<int64_t>(x) : -1;
+  }
+  __device__ static bool next_task(Misc& ms, int& asked, uint32_t& phase, int64_t& task, int* status) {
+    if (!warp_wait(ms, &ms.claimed, phase, status)) return false;
+    --asked;
+    phase ^= 1u;
+    task = answer(ms);
     return true;
+  }
+  __device__ static void note_task(Misc& ms, int64_t task) {
+    if ((threadIdx.x & 31) == 0) ms.taken[ms.n_taken++ % kTaken] = static_cast<uint32_t>(task);
   }
 
   // Tasks (loader 0) and copies until the last task; `issued` counts the ring tiles, `q_issued`
@@ -284,6 +315,7 @@ struct Attend {
           claim_task(ms, asked);
           if (!next_task(ms, asked, cph, task, status)) return;
         }
+        if (t.valid) note_task(ms, task);
         if (!warp_wait(ms, &ms.tempty[tr.i], tr.phase ^ 1u, status)) return;
         if (lane == 0) {
           ms.task[tr.i] = t;
@@ -366,13 +398,27 @@ struct Attend {
     int asked = 0;
     uint32_t cph = 0;
     load_tasks(a, smem, ms, w, issued, q_issued, asked, cph);
-    if (asked > 0) warp_wait(ms, &ms.claimed, cph, a.status);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    for (int i = 0; i < L::kStages && i < issued; ++i) {
-      const int64_t last = issued - 1 - (issued - 1 - i) % L::kStages;      // the last tile put into stage i
-      warp_wait(ms, &ms.kv_full[i], static_cast<uint32_t>(last / L::kStages) & 1u, a.status);
+    const int lane = threadIdx.x & 31;
+    if (asked > 0) {
+      const bool ok = drain_wait(ms, &ms.claimed, cph, a.status);
+      const int64_t task = ok ? answer(ms) : -1;
+      if (task >= 0) note_task(ms, task);
+      if (!ok && lane == 0) ms.lost = 1;
     }
-    if (q_issued > 0) warp_wait(ms, &ms.q_full, static_cast<uint32_t>(q_issued - 1) & 1u, a.status);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // A loader whose wait expired may have left before the others: it arrives for the tiles that they
+    // have issued (fewer than the ring holds, as a stage is filled again only after all arrived for it).
+    if (lane == 0) ms.issued[w] = issued;
+    asm volatile("bar.sync 1, %0;" ::"n"(kLoaders * 32) : "memory");
+    int64_t most = 0;
+    for (int i = 0; i < kLoaders; ++i) most = max(most, ms.issued[i]);
+    for (int64_t i = issued; i < most; ++i) mbar_arrive(&ms.kv_full[i % L::kStages]);
+    __syncwarp();
+    for (int i = 0; i < L::kStages && i < most; ++i) {
+      const int64_t last = most - 1 - (most - 1 - i) % L::kStages;          // the last tile put into stage i
+      drain_wait(ms, &ms.kv_full[i], static_cast<uint32_t>(last / L::kStages) & 1u, a.status);
+    }
+    if (q_issued > 0) drain_wait(ms, &ms.q_full, static_cast<uint32_t>(q_issued - 1) & 1u, a.status);
   }
 
   // ------------------------------------------------------------------ MMA issuer (1 warp)
@@ -426,7 +472,7 @@ struct Attend {
     mma_tasks(a, smem, ms);
     __syncwarp();
     commit(&ms.drain);
-    warp_wait(ms, &ms.drain, 0, a.status);
+    drain_wait(ms, &ms.drain, 0, a.status);
   }
 
   __device__ static void mma_tasks(const AttendLaunch& a, unsigned char* smem, Misc& ms) {
@@ -438,7 +484,7 @@ struct Attend {
     const uint64_t vdesc = smem_desc(smem_addr(smem + L::kOffRing), kHalf, 1024, 2);
     Ring kv, tr;
     uint32_t qph = 0, pph[2] = {0, 0}, oph[2] = {1, 1};
-    while (true) {
+    for (int done = 0; done != a.stall; ++done) {
       if (!warp_wait(ms, &ms.tfull[tr.i], tr.phase, status)) return;
       const AttendTask t = ms.task[tr.i];
       __syncwarp();
@@ -711,8 +757,7 @@ struct Attend {
     const float over_cap = kCap ? a.scale / a.logit_cap : 0.f, cap_log2e = a.logit_cap * kLog2e;
     Ring tr;
     uint32_t sph = 0, oph = 0;
-    bool ok = true;
-    while (ok) {
+    while (true) {
       if (!warp_wait(ms, &ms.tfull[tr.i], tr.phase, status)) return;
       const AttendTask t = ms.task[tr.i];
       __syncwarp();
@@ -728,8 +773,7 @@ struct Attend {
       const int lo = live ? first_key(a, t, row) : 0, hi = live ? last_key(a, t, row) : 0x3fffffff;
       float m = -INFINITY, l = 0.f;
       for (int b = 0; b < blocks; ++b) {
-        ok = warp_wait(ms, &ms.s_full[g], sph, status);
-        if (!ok) break;
+        if (!warp_wait(ms, &ms.s_full[g], sph, status)) return;
         sph ^= 1u;
         tc_fence_after();
         uint32_t s[4][32];
@@ -755,12 +799,12 @@ struct Attend {
           block_after(ms, s_addr, o_addr, c, g, live, b == 0, m, l, s);
       }
       const int64_t at = static_cast<int64_t>(row) * a.query_heads + head;
-      if (blocks > 0 && ok) {
-        ok = warp_wait(ms, &ms.o_full[g], oph, status);
+      if (blocks > 0) {
+        if (!warp_wait(ms, &ms.o_full[g], oph, status)) return;
         oph ^= 1u;
         tc_fence_after();
       }
-      const float inv = !ok ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       const float e2 = l == 0.f ? -INFINITY : m - kBias + lg2(l);
       bool odd = false;
       unsigned char* dst = nullptr;
@@ -778,7 +822,7 @@ struct Attend {
 #pragma unroll 1
         for (int d0 = 0; d0 < D; d0 += 64) {
           uint32_t o[2][32];
-          if (blocks > 0 && ok) {
+          if (blocks > 0) {
             tmem_ld32(o_addr + d0, o[0]);
             tmem_ld32(o_addr + d0 + 32, o[1]);
             tmem_wait32(o[0]);
@@ -797,14 +841,41 @@ struct Attend {
         }
         odd = !(check == 0.f);
         if (live) {
-          const float e = !ok ? inv : e2 * kLn2;
-          if (a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = e;
-          else if (a.lse != nullptr) a.lse[at] = e;
+          if (a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = e2 * kLn2;
+          else if (a.lse != nullptr) a.lse[at] = e2 * kLn2;
         }
       }
-      if (!ok) return;
       const uint32_t again = __ballot_sync(0xffffffffu, odd && live);
-      if (again != 0) form_again<T, D>(a, t, again, row, head, e2, &ms.beat);
+      if (again != 0) form_again<T, D>(a, t, again, row, head, e2, &ms.clock.beat);
+    }
+  }
+
+  // After an expired wait, by the softmax warps: NaN for the rows (and split results) of the last tasks
+  // taken, as no other CTA will run them.  Some may have been stored in full: they are NaN all the same.
+  // Where the hardware did not answer a claim, the task is not known, and every row of the call is set.
+  __device__ static void give_up(const AttendLaunch& a, const Misc& ms) {
+    const int warp = (threadIdx.x >> 5) - kSoftmaxWarp, lane = threadIdx.x & 31;
+    const int tokens = kRows / a.group;
+    const float nan = __int_as_float(0x7fc00000);
+    const uint32_t n = ms.lost ? gridDim.x : min(ms.n_taken, static_cast<uint32_t>(kTaken));
+    int chunk = 0;
+    int64_t before = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+      const AttendTask t = find_task(a, 2 * tokens, kRows, ms.lost ? i : ms.taken[i], chunk, before);
+      if (!t.valid) continue;
+      for (int r = warp; r < (t.last - t.first) * a.group; r += kWarps - kSoftmaxWarp) {
+        const int row = t.first + r / a.group, head = t.head * a.group + r % a.group;
+        const int64_t at = static_cast<int64_t>(row) * a.query_heads + head;
+        for (int d = lane; d < D; d += 32) {
+          if (a.partial != nullptr)
+            a.partial[(at * a.splits + t.split) * D + d] = nan;
+          else
+            static_cast<T*>(a.out)[static_cast<int64_t>(row) * a.out_stride[0] + static_cast<int64_t>(head) * a.out_stride[1] + d] =
+                from_float<T>(nan);
+        }
+        if (lane == 0 && a.partial != nullptr) a.partial_lse[at * a.splits + t.split] = nan;
+        else if (lane == 0 && a.lse != nullptr) a.lse[at] = nan;
+      }
     }
   }
 };
@@ -818,7 +889,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   Misc& ms = *reinterpret_cast<Misc*>(smem + L::kOffMisc);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    ms.beat = 0;
+    ms.clock = Clock{0, a.wait_ns};
+    ms.drain_clock = Clock{0, kDrainLimitNs};
+    ms.n_taken = ms.lost = 0;
     for (int i = 0; i < L::kStages; ++i) mbar_init(&ms.kv_full[i], kLoaders * 32), mbar_init(&ms.kv_empty[i], 1);
     mbar_init(&ms.q_full, 1), mbar_init(&ms.q_empty, 1), mbar_init(&ms.drain, 1), mbar_init(&ms.claimed, 1);
     for (int g = 0; g < 2; ++g)
@@ -845,6 +918,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) tmem_dealloc(ms.tmem_base, kTmemCols);
+  if (warp >= kSoftmaxWarp && (ms.clock.beat == kFailed || ms.lost)) A::give_up(a, ms);
 }
 
 template <typename T, int D, bool kCap>

@@ -143,6 +143,17 @@ bool tma_disabled_by_env() {
 // whole call is in flight at once; above it four, which reads the rotation once for four steps.
 constexpr int64_t kFewRopeSteps = 148 * 64;
 
+// SGLD_ATTEND_STALL=tasks:ns makes waits of the tcgen05 attention kernel run out, for tests: its issuer stops
+// after that many tasks in every CTA (-1: never), and waits expire after that many ns, not 4 s.
+void set_wait_limits(sgld::AttendLaunch& a) {
+  a.stall = -1;
+  a.wait_ns = 4000000000ull;
+  const char* v = std::getenv("SGLD_ATTEND_STALL");
+  int stall = 0;
+  unsigned long long ns = 0;
+  if (v != nullptr && std::sscanf(v, "%d:%llu", &stall, &ns) == 2) a.stall = stall < -1 ? -1 : stall, a.wait_ns = ns;
+}
+
 int check_plan_pointers(const sgld_plan_buffers* p) {
   if (p == nullptr) return fail(SGLD_ERR_INVALID_ARGUMENT, "plan buffers are NULL");
   const void* ptrs[] = {p->lengths, p->splits, p->active, p->counts, p->offsets, p->chunk,
@@ -566,6 +577,7 @@ bool pool_maps(const sgld::AttendLaunch& a, const void* base, const int64_t* str
 
 // Row alignment and, where the tcgen05 kernel applies, its tensor maps (true).
 bool prepare_attend(sgld::AttendLaunch& a) {
+  set_wait_limits(a);
   // The stride of an extent of one is never used: any value may stand there.
   if (a.tokens == 1) a.q_stride[0] = a.out_stride[0] = static_cast<int64_t>(a.query_heads) * a.head_dim;
   if (a.query_heads == 1) a.q_stride[1] = a.out_stride[1] = a.head_dim;

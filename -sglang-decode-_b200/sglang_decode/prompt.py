@@ -29,7 +29,8 @@ def prompt_attention(q, k, v, indptr, *, kv_indptr=None, kv_indices=None, scale=
     reaches the rows that see it and no others.  Rows of ``out`` (allocated when absent; it must not
     share memory with the inputs) outside the sequences are left as they were.  ``lse`` (fp32 [T, Hq], optional) receives
     each row's natural-log sum of exponentials, -inf without a key; ``status`` (int32[1], optional)
-    is set non-zero if an in-kernel wait expires (rows are then NaN).
+    is set non-zero if an in-kernel wait expires (4 s; every row that this kept from being computed is then
+    NaN, and some of the same thread block's others).
 
     Scores, softmax and sums are fp32; the weights are rounded to q's dtype for their product with
     ``v``.  Returns ``out``.

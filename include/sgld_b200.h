@@ -294,7 +294,8 @@ typedef struct sgld_prompt_args {
   const int32_t* kv_indptr; /* [seqs + 1]; NULL: q_indptr                                       */
   const int32_t* kv_indices;/* [kv_indices_count] rows of k / v, one per key; NULL: key j of a
                                sequence is row kv_indptr[i] + j.  A row outside k reads as zeros */
-  int32_t* status;          /* [1] sticky bit 1: a bounded in-kernel wait expired; or NULL      */
+  int32_t* status;          /* [1] sticky bit 1: a bounded in-kernel wait expired (rows kept from
+                               being computed are NaN, with or without a status word); or NULL  */
   int64_t q_stride[3];      /* elements: (token, head, dim)                                     */
   int64_t k_stride[3];
   int64_t v_stride[3];
