@@ -234,8 +234,8 @@ cudaError_t launch_dim(const AttendLaunch& a, cudaStream_t stream) {
 // for the prompt attention, and for a decode without an index of own tokens, whose rows with counts
 // are NaN), each in split order.  A slot whose LSE is -inf saw no key: its values do not count.  A row is a chain of two memory round trips (its count, its slots), which bound the
 // kernel, not the bytes: values are loaded together with their LSEs, four slots at a time, at 64
-// registers for 32 warps an SM (16384 rows of 3 slots: 23 us; with eight slots and their values only
-// after the LSEs, at 96 registers, 34).
+// registers for 32 warps an SM (16384 rows of nine prefix slots and one own: 23 us; with eight slots at a
+// time and their values only after the LSEs, at 96 registers, 34).
 struct MergeLaunch {
   const float* first;
   const float* first_lse;
