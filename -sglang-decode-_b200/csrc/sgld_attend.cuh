@@ -311,8 +311,9 @@ __device__ __forceinline__ float capped_log2(float s, float scale_over_cap, floa
 // question is asked of all rows together: the keys that all of them see are searched once, from the
 // newest (a bad token is mostly followed by bad ones) until NaNs settle every value in question.
 // Rows that need the sum are those beside a bad value that they do not see: one or two tiles of a
-// sequence for each dim.  One NaN among the first keys of 32 / 8 heads: 0.28 ms for
-// 1024 tokens (57 when each row walked its own keys one by one), 4.9 for 8192.
+// sequence for each dim.  One NaN among the first keys of 32 / 8 heads: 0.26 ms for
+// 1024 tokens (57 when each row walked its own keys one by one), 3.7 for 8192.  The last of 16000 tokens NaN, 16 / 4
+// heads, so that the 63 before it in its tile are summed again: 29 ms.
 //
 // A row of V or K is D / 8 lanes of 16 bytes; a warp reads 256 / D keys at a time.
 struct Kinds {             // bit i: the lane's dim i has a NaN, a plus or a minus infinity
@@ -358,13 +359,15 @@ __device__ __forceinline__ int64_t row_offset(const AttendLaunch& a, const int64
 
 // The values that are not finite in V of keys [from, to), newest first, until `want` of the lane's dims are
 // all known to hold a NaN; whole warp, the same in all lanes of a dim.
-template <typename T, int D>
+template <typename T, int D, int R>
 __device__ __forceinline__ void find_kinds(const AttendLaunch& a, const AttendTask& t, int from, int to, uint32_t want,
                                            Kinds& k, uint64_t* beat) {
   constexpr int kLanes = D / 8, kSub = 32 / kLanes, kAhead = 4;
   constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u, kExp2 = kExp | kExp << 16;
   const int lane = threadIdx.x & 31, sub = lane / kLanes;
-  const T* v = static_cast<const T*>(a.v) + t.head * a.v_stride[2] + (lane % kLanes) * 8 * a.v_stride[3];
+  const int64_t stride = a.v_stride[3];
+  const bool aligned = R > 1 || a.aligned != 0;       // (always in the tcgen05 kernel)
+  const T* v = static_cast<const T*>(a.v) + t.head * a.v_stride[2] + (lane % kLanes) * 8 * stride;
   for (int end = to; end > from; end -= 32) {
     if (__all_sync(0xffffffffu, (k.nan & want) == want)) return;
     const int64_t mine = end - 1 - lane >= from ? row_offset(a, a.v_stride, key_slot(a, t.kv_begin, end - 1 - lane)) : -1;
@@ -374,7 +377,7 @@ __device__ __forceinline__ void find_kinds(const AttendLaunch& a, const AttendTa
       for (int i = 0; i < kAhead; ++i) {
         const int64_t at = __shfl_sync(0xffffffffu, mine, (u + i) * kSub + sub);
         w[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (at >= 0) w[i] = load_dims<T>(v + at, a.v_stride[3], a.aligned != 0);
+        if (at >= 0) w[i] = load_dims<T>(v + at, stride, aligned);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -402,22 +405,36 @@ __device__ __forceinline__ void find_kinds(const AttendLaunch& a, const AttendTa
   }
 }
 
-// The lane's dims of sum_j p_j v_j / sum_j p_j over keys [from, to), by one warp; p_j = 2^(s_j - e2), e2 the row's
-// log2-sum-exp, so that the p_j sum to about one and no partial sum exceeds the largest value.
-template <typename T, int D>
-__device__ __forceinline__ void sum_again(const AttendLaunch& a, const AttendTask& t, int row, int head, int from, int to,
-                                          float e2, float (&acc)[8], uint64_t* beat) {
+// The lane's dims of sum_j p_j v_j / sum_j p_j for up to R rows at once, by one warp; row i: token row[i], query
+// head head[i], keys [from[i], to[i]) (from >= to: no such row).  p_j = 2^(s_j - e2), e2 the row's log2-sum-exp, so that
+// the p_j sum to about one and no partial sum exceeds the largest value.  Rows share the loads, whose latency
+// bounds it: four in the tcgen05 kernel, one in the mma.sync kernel, which has no registers for more.
+template <typename T, int D, int R>
+__device__ __forceinline__ void sum_again(const AttendLaunch& a, const AttendTask& t, const int (&row)[R],
+                                          const int (&head)[R], const int (&from)[R], const int (&to)[R],
+                                          const float (&e2)[R], float (&acc)[R][8], uint64_t* beat) {
   constexpr int kLanes = D / 8, kSub = 32 / kLanes, kAhead = 4;
   const int lane = threadIdx.x & 31, sub = lane / kLanes, d0 = (lane % kLanes) * 8;
-  float q[8], sum = 0.f;
-  to_dims<T>(load_dims<T>(static_cast<const T*>(a.q) + static_cast<int64_t>(row) * a.q_stride[0] +
-                              static_cast<int64_t>(head) * a.q_stride[1] + d0 * a.q_stride[2], a.q_stride[2], a.aligned != 0), q);
+  const int64_t ks = a.k_stride[3], vs = a.v_stride[3];
+  const bool aligned = R > 1 || a.aligned != 0;
+  float q[R][8], sum[R];
+  int first = 0x7fffffff, end = 0;
 #pragma unroll
-  for (int x = 0; x < 8; ++x) acc[x] = 0.f;
-  const T* k = static_cast<const T*>(a.k) + t.head * a.k_stride[2] + d0 * a.k_stride[3];
-  const T* v = static_cast<const T*>(a.v) + t.head * a.v_stride[2] + d0 * a.v_stride[3];
-  for (int j0 = from; j0 < to; j0 += 32) {
-    const int64_t slot = j0 + lane < to ? key_slot(a, t.kv_begin, j0 + lane) : -1;
+  for (int i = 0; i < R; ++i) {
+    sum[i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) q[i][x] = acc[i][x] = 0.f;
+    if (from[i] >= to[i]) continue;
+    first = min(first, from[i]);
+    end = max(end, to[i]);
+    to_dims<T>(load_dims<T>(static_cast<const T*>(a.q) + static_cast<int64_t>(row[i]) * a.q_stride[0] +
+                                static_cast<int64_t>(head[i]) * a.q_stride[1] + d0 * a.q_stride[2], a.q_stride[2], aligned), q[i]);
+  }
+  const T* k = static_cast<const T*>(a.k) + t.head * a.k_stride[2] + d0 * ks;
+  const T* v = static_cast<const T*>(a.v) + t.head * a.v_stride[2] + d0 * vs;
+  const float scale = a.scale * 1.4426950408889634f, cap = a.logit_cap, over_cap = cap > 0.f ? a.scale / cap : 0.f;
+  for (int j0 = first; j0 < end; j0 += 32) {
+    const int64_t slot = j0 + lane < end ? key_slot(a, t.kv_begin, j0 + lane) : -1;
     const int64_t my_k = row_offset(a, a.k_stride, slot), my_v = row_offset(a, a.v_stride, slot);
     for (int u = 0; u < kLanes; u += kAhead) {
       uint4 kw[kAhead], vw[kAhead];
@@ -427,42 +444,64 @@ __device__ __forceinline__ void sum_again(const AttendLaunch& a, const AttendTas
         const int64_t at_v = __shfl_sync(0xffffffffu, my_v, (u + i) * kSub + sub);
         kw[i] = vw[i] = make_uint4(0u, 0u, 0u, 0u);
         if (at_k >= 0) {
-          kw[i] = load_dims<T>(k + at_k, a.k_stride[3], a.aligned != 0);
-          vw[i] = load_dims<T>(v + at_v, a.v_stride[3], a.aligned != 0);
+          kw[i] = load_dims<T>(k + at_k, ks, aligned);
+          vw[i] = load_dims<T>(v + at_v, vs, aligned);
         }
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        float x[8], s = 0.f;
-        to_dims<T>(kw[i], x);
+        const int j = j0 + (u + i) * kSub + sub;
+        float kx[8], vx[8], sc[R];
+        to_dims<T>(kw[i], kx);
+        to_dims<T>(vw[i], vx);
+        // (A value that is not finite counts for no row: those that see it do not ask for its dim.)
 #pragma unroll
-        for (int y = 0; y < 8; ++y) s = fmaf(q[y], x[y], s);
+        for (int y = 0; y < 8; ++y) vx[y] = fabsf(vx[y]) <= 3.4028235e38f ? vx[y] : 0.f;
 #pragma unroll
-        for (int bit = kLanes / 2; bit >= 1; bit >>= 1) s += __shfl_xor_sync(0xffffffffu, s, bit);
-        s = a.logit_cap > 0.f ? capped_log2(s, a.scale / a.logit_cap, a.logit_cap * 1.4426950408889634f)
-                              : s * (a.scale * 1.4426950408889634f);
-        const float p = j0 + (u + i) * kSub + sub < to ? ex2(s - e2) : 0.f;
-        sum += p;
-        to_dims<T>(vw[i], x);
+        for (int r = 0; r < R; ++r) {
+          sc[r] = 0.f;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) acc[y] = fmaf(p, x[y], acc[y]);
+          for (int y = 0; y < 8; ++y) sc[r] = fmaf(q[r][y], kx[y], sc[r]);
+        }
+#pragma unroll
+        for (int bit = kLanes / 2; bit >= 1; bit >>= 1) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) sc[r] += __shfl_xor_sync(0xffffffffu, sc[r], bit);
+        }
+        if (cap > 0.f) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) sc[r] = capped_log2(sc[r], over_cap, cap * 1.4426950408889634f);
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r) sc[r] *= scale;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float w = ex2(sc[r] - e2[r]), p = j >= from[r] && j < to[r] ? w : 0.f;
+          sum[r] += p;
+#pragma unroll
+          for (int y = 0; y < 8; ++y) acc[r][y] = fmaf(p, vx[y], acc[r][y]);
+        }
       }
     }
     take_time(beat);
   }
 #pragma unroll
-  for (int bit = kLanes; bit < 32; bit <<= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+  for (int r = 0; r < R; ++r) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] += __shfl_xor_sync(0xffffffffu, acc[x], bit);
+    for (int bit = kLanes; bit < 32; bit <<= 1) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], bit);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[r][x] += __shfl_xor_sync(0xffffffffu, acc[r][x], bit);
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[r][x] /= sum[r];
   }
-#pragma unroll
-  for (int x = 0; x < 8; ++x) acc[x] /= sum;
 }
 
 // `odd`: the lanes whose row (token `row`, query head `head`, log2-sum-exp `e2`) has a stored result that is not finite.
 // `beat` (shared memory, or nullptr): the time of the last step, for waits that stand behind this one.
-template <typename T, int D>
+template <typename T, int D, int R>
 __device__ __noinline__ void form_again(const AttendLaunch& a, const AttendTask& t, uint32_t odd, int row, int head, float e2,
                                         uint64_t* beat) {
   constexpr int kLanes = D / 8;
@@ -471,10 +510,18 @@ __device__ __noinline__ void form_again(const AttendLaunch& a, const AttendTask&
   // (A sum that is not finite comes from a score that is NaN, and with it the whole row stays so.)
   odd = __ballot_sync(0xffffffffu, (odd >> lane & 1u) != 0 && (e2 == -INFINITY || fabsf(e2) <= 3.4028235e38f));
   const bool mine = (odd >> lane & 1u) != 0 && e2 != -INFINITY;
-  const auto result = [&](int64_t at_row, int at_head, int x) -> float {
+  const auto bad_dims = [&](int64_t at_row, int at_head) -> uint32_t {   // of a row's stored result
     const int64_t at = at_row * a.query_heads + at_head;
-    if (a.partial != nullptr) return a.partial[(at * a.splits + t.split) * D + d0 + x];
-    return to_float<T>(static_cast<const T*>(a.out)[at_row * a.out_stride[0] + at_head * a.out_stride[1] + (d0 + x) * a.out_stride[2]]);
+    uint32_t bad = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float y = a.partial != nullptr
+                          ? a.partial[(at * a.splits + t.split) * D + d0 + x]
+                          : to_float<T>(static_cast<const T*>(a.out)[at_row * a.out_stride[0] + at_head * a.out_stride[1] +
+                                                                     (d0 + x) * a.out_stride[2]]);
+      bad |= (fabsf(y) <= 3.4028235e38f ? 0u : 1u) << x;
+    }
+    return bad;
   };
   // The keys that all of these rows see, and the dims that any of them asks for.
   int from = __reduce_max_sync(0xffffffffu, mine ? first_key(a, t, row) : 0);
@@ -482,46 +529,62 @@ __device__ __noinline__ void form_again(const AttendLaunch& a, const AttendTask&
   if (from >= to) from = to = t.lo;                   // (none: each row looks through its own)
   uint32_t any = 0;
   for (uint32_t rest = odd; rest != 0; rest &= rest - 1) {
-    const int who = __ffs(rest) - 1, r = __shfl_sync(0xffffffffu, row, who), h = __shfl_sync(0xffffffffu, head, who);
-#pragma unroll
-    for (int x = 0; x < 8; ++x) any |= (fabsf(result(r, h, x)) <= 3.4028235e38f ? 0u : 1u) << x;
+    const int who = __ffs(rest) - 1;
+    any |= bad_dims(__shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, head, who));
   }
   Kinds common;
   bool searched = false;
-  for (; odd != 0; odd &= odd - 1) {
-    const int who = __ffs(odd) - 1, r = __shfl_sync(0xffffffffu, row, who), h = __shfl_sync(0xffffffffu, head, who);
-    const float e = __shfl_sync(0xffffffffu, e2, who);
-    uint32_t want = 0;
+  while (odd != 0) {
+    int rows[R], heads[R], lo[R], hi[R];
+    float e[R], acc[R][8] = {};
+    uint32_t want[R];
+    Kinds k[R];
+    bool sum = false;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) want |= (fabsf(result(r, h, x)) <= 3.4028235e38f ? 0u : 1u) << x;
-    Kinds k;
-    float acc[8] = {};
-    if (e != -INFINITY) {                             // (a row without a weight is zero)
-      if (!searched) find_kinds<T, D>(a, t, from, to, any, common, beat);
+    for (int i = 0; i < R; ++i) {
+      want[i] = 0;
+      lo[i] = hi[i] = rows[i] = heads[i] = 0;
+      e[i] = 0.f;
+      if (odd == 0) continue;
+      const int who = __ffs(odd) - 1;
+      odd &= odd - 1;
+      rows[i] = __shfl_sync(0xffffffffu, row, who);
+      heads[i] = __shfl_sync(0xffffffffu, head, who);
+      e[i] = __shfl_sync(0xffffffffu, e2, who);
+      want[i] = bad_dims(rows[i], heads[i]);
+      if (e[i] == -INFINITY) continue;                // a row without a weight is zero
+      if (!searched) find_kinds<T, D, R>(a, t, from, to, any, common, beat);
       searched = true;
-      k = common;
-      const int lo = first_key(a, t, r), hi = last_key(a, t, r) + 1;
+      k[i] = common;
+      lo[i] = first_key(a, t, rows[i]);
+      hi[i] = last_key(a, t, rows[i]) + 1;
       if (from < to) {
-        find_kinds<T, D>(a, t, lo, from, want, k, beat);
-        find_kinds<T, D>(a, t, to, hi, want, k, beat);
+        find_kinds<T, D, R>(a, t, lo[i], from, want[i], k[i], beat);
+        find_kinds<T, D, R>(a, t, to, hi[i], want[i], k[i], beat);
       } else {
-        find_kinds<T, D>(a, t, lo, hi, want, k, beat);
+        find_kinds<T, D, R>(a, t, lo[i], hi[i], want[i], k[i], beat);
       }
-      if (__any_sync(0xffffffffu, (want & ~(k.nan | k.up | k.down)) != 0)) sum_again<T, D>(a, t, r, h, lo, hi, e, acc, beat);
+      if (__any_sync(0xffffffffu, (want[i] & ~(k[i].nan | k[i].up | k[i].down)) != 0)) sum = true;
+      else hi[i] = lo[i];
     }
+    if (sum) sum_again<T, D, R>(a, t, rows, heads, lo, hi, e, acc, beat);
     if (lane >= kLanes) continue;
-    const int64_t at = static_cast<int64_t>(r) * a.query_heads + h;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const uint32_t bit = 1u << x;
-      if (!(want & bit)) continue;
-      const float y = (k.nan & bit) || ((k.up & bit) && (k.down & bit)) ? __int_as_float(0x7fc00000)
-                      : (k.up & bit) ? INFINITY : (k.down & bit) ? -INFINITY : acc[x];
-      if (a.partial != nullptr) {
-        a.partial[(at * a.splits + t.split) * D + d0 + x] = y;
-      } else {
-        static_cast<T*>(a.out)[static_cast<int64_t>(r) * a.out_stride[0] + static_cast<int64_t>(h) * a.out_stride[1] +
-                               (d0 + x) * a.out_stride[2]] = from_float<T>(y);
+    for (int i = 0; i < R; ++i) {
+      const int64_t at = static_cast<int64_t>(rows[i]) * a.query_heads + heads[i];
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t bit = 1u << x;
+        if (!(want[i] & bit)) continue;
+        const float y = e[i] == -INFINITY ? 0.f
+                        : (k[i].nan & bit) || ((k[i].up & bit) && (k[i].down & bit)) ? __int_as_float(0x7fc00000)
+                        : (k[i].up & bit) ? INFINITY : (k[i].down & bit) ? -INFINITY : acc[i][x];
+        if (a.partial != nullptr) {
+          a.partial[(at * a.splits + t.split) * D + d0 + x] = y;
+        } else {
+          static_cast<T*>(a.out)[static_cast<int64_t>(rows[i]) * a.out_stride[0] + static_cast<int64_t>(heads[i]) * a.out_stride[1] +
+                                 (d0 + x) * a.out_stride[2]] = from_float<T>(y);
+        }
       }
     }
   }

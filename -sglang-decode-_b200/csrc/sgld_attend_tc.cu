@@ -23,7 +23,7 @@
 // 16 a cycle), so the two run at the same pace and overlap; K and V come through L2.  Measured: 3550
 // cycles, a tile's chain of softmax (2000) and P V, Q K and their latencies (1280) with two tiles in
 // flight, which is what tensor memory holds (S 2 x 128 + O 2 x 128 columns): two causal prompts of
-// 8K tokens, 32 / 8 heads, D 128: 1003-1039 us with the power cap's clock, 1.03-1.07 PFLOP/s.
+// 8K tokens, 32 / 8 heads, D 128: 1003-1048 us with the power cap's clock, 1.03-1.07 PFLOP/s.
 //
 // Precision: scores, maxima, sums and O are fp32; p is rounded to 16 bits for the second product
 // (its operand type), the sum keeps the fp32 values.
@@ -846,7 +846,7 @@ struct Attend {
         }
       }
       const uint32_t again = __ballot_sync(0xffffffffu, odd && live);
-      if (again != 0) form_again<T, D>(a, t, again, row, head, e2, &ms.clock.beat);
+      if (again != 0) form_again<T, D, 4>(a, t, again, row, head, e2, &ms.clock.beat);
     }
   }
 

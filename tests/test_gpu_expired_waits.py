@@ -69,7 +69,7 @@ def test_shared_prefix(cuda_device, monkeypatch, page):
 
 def test_waits_behind_rows_that_are_formed_again_go_on(cuda_device, monkeypatch):
     """The last 63 other tokens of each head see 16000 finite keys beside a masked NaN: a warp sums 32 of such
-    rows for a tenth of a second, and the waits expire after a millisecond without a step of it."""
+    rows for some 30 ms, and the waits expire after a millisecond without a step of it."""
     q, k, v, kv, index = case([16000], [0], 16, 4, 128, BF, False)
     clean = prompt_attention(q, k, v, pointers([16000]))
     v[15999] = float("nan")
